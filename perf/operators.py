@@ -568,7 +568,7 @@ def _own_prologue(s):
     q = ops.gqa_draft_prologue(s["q"], s["k_new"], s["v_new"], s["q_norm"], s["k_norm"], s["cos"], s["sin"], s["k"], s["k_scales"], s["v"], s["v_scales"],
                                s["tables"], s["kv_lens"], case["heads"], case["kv_heads"], case["dim"], case["rotary"], case["page"], positions=s["positions"],
                                row_counts=s["counts"], split_half=case["layout"] == "half", q_out_dtype=_DTYPES[case["dtype"]],
-                               rule=capi.QUANT_RECIPROCAL_GQA, kv_format=capi.KV_F16 if f16 else capi.KV_Q8G64)
+                               kv_format=capi.KV_F16 if f16 else capi.KV_Q8G64)
     return {"q": q, "k": s["k"], "v": s["v"]} if f16 else {"q": q, "k": s["k"], "k_scales": s["k_scales"], "v": s["v"], "v_scales": s["v_scales"]}
 
 
