@@ -57,8 +57,14 @@ enum { ZLLM_KV_Q8G64 = 0, ZLLM_KV_F16 = 1 };
  *              nearbyint(x / f32(stored))   (paged_mla/source.hip:183-201)
  *   METAL_GQA: scale = absmax / 127 (1.0 if 0), stored f16, codes =
  *              rint(x * (1 / scale))        (kernel/metal/attention/mod.rs:114-127)
- *   CUDA_GQA : as METAL_GQA, stored f32     (kernel/cuda/attention.rs:331-341) */
-enum { ZLLM_QUANT_ROCM_MLA = 0, ZLLM_QUANT_METAL_GQA = 1, ZLLM_QUANT_CUDA_GQA = 2 };
+ *   CUDA_GQA : as METAL_GQA, stored f32     (kernel/cuda/attention.rs:331-341)
+ * and one that has no counterpart there:
+ *   RECIPROCAL_GQA: METAL_GQA with its divisions by a constant (absmax / 127, and a prologue's mean over head_dim) as
+ *              products with the rounded reciprocal, which is how tensor programs on GPUs divide by a constant: the
+ *              bits that such a program writes.  They differ from METAL_GQA's in the last bit of a scale before it is
+ *              stored and in codes that lie on a tie (50 of a million with bf16 values); either row is within half a
+ *              step, and a cache may hold both.  Whoever needs the bits of another writer's rows names that writer's rule. */
+enum { ZLLM_QUANT_ROCM_MLA = 0, ZLLM_QUANT_METAL_GQA = 1, ZLLM_QUANT_CUDA_GQA = 2, ZLLM_QUANT_RECIPROCAL_GQA = 3 };
 
 /* RoPE pair layout (src/attention/rope.rs:106-110). */
 enum { ZLLM_ROTARY_INTERLEAVED = 0, ZLLM_ROTARY_SPLIT_HALF = 1 };
@@ -560,12 +566,6 @@ typedef struct zllm_draft_layout_args {
 } zllm_draft_layout_args;
 ZLLM_API int zllm_attn_draft_layout(const zllm_draft_layout_args* args, zllm_stream_t stream);
 
-/* A rule of zllm_attn_gqa_draft_prologue beside ZLLM_QUANT_*: METAL_GQA with its divisions by a constant (absmax / 127, and the
- * norm's mean over head_dim) as products with the rounded reciprocal, which is how array libraries on GPUs divide by a
- * constant.  Its rows are bit for bit those of a cache that such code writes; they differ from METAL_GQA's in the last bit
- * of a scale and in codes that lie on a tie. */
-enum { ZLLM_QUANT_RECIPROCAL_GQA = 3 };
-
 /* zllm_attn_gqa_prologue for the drafted nodes of a batch: row b * rows + i rotates at positions[b, i] (NULL: a chain,
  * kv_lens[b] + i) and its K and V go to cache token kv_lens[b] + i of sequence b, as Q8g64 or as f16 rows.  Same arithmetic,
  * same bits.  Nodes that are not there get a zero query and write nothing to the cache; neither does a node behind the
@@ -597,7 +597,7 @@ typedef struct zllm_gqa_draft_prologue_args {
     int src_dtype;              /* ZLLM_DTYPE_* of q, k, v */
     int q_out_dtype;            /* ZLLM_DTYPE_* */
     int kv_format;              /* ZLLM_KV_* */
-    int rule;                   /* ZLLM_QUANT_* or ZLLM_QUANT_RECIPROCAL_GQA */
+    int rule;                   /* ZLLM_QUANT_* */
     int split_half;             /* 1 = pairs (i, i + rotary_dim / 2), 0 = interleaved (2 i, 2 i + 1) */
 } zllm_gqa_draft_prologue_args;
 ZLLM_API int zllm_attn_gqa_draft_prologue(const zllm_gqa_draft_prologue_args* args, zllm_stream_t stream);

@@ -712,3 +712,46 @@ def test_two_streams_at_once():
             assert torch.equal(out, want[i])
         for out in got_verify[i]:
             assert all(torch.equal(a, b) for a, b in zip(out, want_verify[i]))
+
+
+def test_prologue_default_rows_are_those_of_a_tensor_program():
+    """The entry point's own quantizer: the bits that the formula has where a tensor program on this device evaluates it, with bf16 and f16 values whose groups
+    have ordinary maxima (half a maximum lies on a tie of two codes).  METAL_GQA at the same values has the bits of the prologue and the append of single
+    sequences, and so has RECIPROCAL_GQA, which those take as well."""
+    gen = torch.Generator().manual_seed(77)
+    batch, rows, heads, d, page = 24, 48, 8, 128, 16
+    nodes, cols = batch * rows, heads * d
+    tables = torch.randperm(batch * 3, generator=gen).to(torch.int32).view(batch, 3)
+    slots = (tables.long()[..., None] * page + torch.arange(page)).view(batch * rows).cuda()
+    norm = (torch.randn(d, generator=gen) * 0.1).cuda()
+    for src in (torch.bfloat16, torch.float16, torch.float32):
+        q, k, v = torch.randn(3, nodes, cols, generator=gen).to(src).cuda()
+        empty = lambda: [torch.zeros(nodes, cols, dtype=torch.int8, device="cuda"), torch.zeros(nodes, cols // 64, dtype=torch.float16, device="cuda")] * 1
+
+        def drafted(**rule):
+            planes = empty() + empty()
+            out = ops.gqa_draft_prologue(q, k, v, norm, norm, None, None, *planes, dev(tables), ints([0] * batch), heads, heads, d, 0, page, **rule)
+            return out, [p[slots] for p in planes]
+
+        out, (k_codes, k_scales, v_codes, v_scales) = drafted()
+        groups = v.float().view(nodes, -1, 64)
+        most = groups.abs().amax(-1)
+        step = most / 127.0
+        assert torch.equal(step, most * torch.tensor(1.0 / 127.0, device="cuda"))
+        assert torch.equal(v_scales, step.half())
+        assert torch.equal(v_codes.view(groups.shape), torch.round(groups * (1.0 / step)[..., None]).clamp(-127, 127).to(torch.int8))
+        results = {}
+        for rule in (capi.QUANT_METAL_GQA, capi.QUANT_RECIPROCAL_GQA):
+            results[rule] = drafted(rule=rule)
+            single = empty() + empty()
+            single_out = ops.gqa_prologue(q, k, v, norm, norm, None, None, *single, None, 0, heads, heads, d, 0, page, rule=rule)
+            assert torch.equal(single_out, results[rule][0])
+            for one, other in zip(single, results[rule][1]):
+                assert torch.equal(one, other)
+            appended = empty()
+            ops.q8g64_append(v, *appended, None, 0, page, rule)
+            assert torch.equal(appended[0], single[2]) and torch.equal(appended[1], single[3])
+        for one, other in zip([out, k_codes, k_scales, v_codes, v_scales], [results[capi.QUANT_RECIPROCAL_GQA][0], *results[capi.QUANT_RECIPROCAL_GQA][1]]):
+            assert torch.equal(one, other)
+        if src == torch.bfloat16:  # the two rules do differ here
+            assert not torch.equal(results[capi.QUANT_METAL_GQA][1][2], v_codes)

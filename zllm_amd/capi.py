@@ -16,7 +16,7 @@ SCALE_BF16, SCALE_F16, SCALE_F32 = 0, 1, 2
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 KV_Q8G64, KV_F16 = 0, 1
 QUANT_ROCM_MLA, QUANT_METAL_GQA, QUANT_CUDA_GQA = 0, 1, 2
-QUANT_RECIPROCAL_GQA = 3  # gqa_draft_prologue: METAL_GQA as array libraries compute it
+QUANT_RECIPROCAL_GQA = 3  # METAL_GQA as tensor programs compute it: products with 1 / 127 and 1 / head_dim
 ROTARY_INTERLEAVED, ROTARY_SPLIT_HALF = 0, 1
 STAGE_ALL, STAGE_PARTIAL, STAGE_MERGE = 0, 1, 2
 MLA_ABSORB, MLA_PARTIAL, MLA_MERGE, MLA_PROJECT = 1, 2, 4, 8

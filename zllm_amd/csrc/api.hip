@@ -649,7 +649,7 @@ int zllm_attn_q8g64_append(const zllm_q8_append_args* a, zllm_stream_t stream)
     if (a->cols == 0 || a->cols % ZLLM_GROUP_SIZE != 0 || a->block_tokens == 0) {
         return fail(-1, "Q8g64 append: cols=%u must be a non-zero multiple of 64, block_tokens=%u non-zero", a->cols, a->block_tokens);
     }
-    if (a->rule < ZLLM_QUANT_ROCM_MLA || a->rule > ZLLM_QUANT_CUDA_GQA || a->src_dtype < ZLLM_DTYPE_F32 || a->src_dtype > ZLLM_DTYPE_F16) {
+    if (a->rule < ZLLM_QUANT_ROCM_MLA || a->rule > ZLLM_QUANT_RECIPROCAL_GQA || a->src_dtype < ZLLM_DTYPE_F32 || a->src_dtype > ZLLM_DTYPE_F16) {
         return fail(-1, "Q8g64 append: unknown rule %d or src_dtype %d", a->rule, a->src_dtype);
     }
     if ((uint64_t)a->position + a->rows > 0xffffffffull) {
@@ -681,7 +681,7 @@ int zllm_attn_gqa_prologue(const zllm_gqa_prologue_args* a, zllm_stream_t stream
     if ((a->q_norm != nullptr || a->k_norm != nullptr) && !(a->eps > 0.0f && a->eps < INFINITY)) {
         return fail(-1, "GQA prologue: eps must be finite and positive");
     }
-    if (a->rule < ZLLM_QUANT_ROCM_MLA || a->rule > ZLLM_QUANT_CUDA_GQA || a->src_dtype < ZLLM_DTYPE_F32 || a->src_dtype > ZLLM_DTYPE_F16 ||
+    if (a->rule < ZLLM_QUANT_ROCM_MLA || a->rule > ZLLM_QUANT_RECIPROCAL_GQA || a->src_dtype < ZLLM_DTYPE_F32 || a->src_dtype > ZLLM_DTYPE_F16 ||
         (a->q_out_dtype != ZLLM_DTYPE_F32 && a->q_out_dtype != ZLLM_DTYPE_BF16)) {
         return fail(-1, "GQA prologue: unknown rule %d, src_dtype %d or q_out_dtype %d", a->rule, a->src_dtype, a->q_out_dtype);
     }

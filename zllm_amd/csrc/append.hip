@@ -32,7 +32,7 @@ __device__ __forceinline__ float wave_max_all(float v)
 //   rule 1 (kernel/metal/attention/mod.rs:114-127): scale = absmax / 127,
 //          stored f16, code = rint(x * (1 / scale)).
 //   rule 2 (kernel/cuda/attention.rs:331-341): as rule 1, stored f32.
-//   rule 3: as rule 1 with absmax * (1/127) for absmax / 127 (drafted nodes only).
+//   rule 3: as rule 1 with absmax * (1/127) for absmax / 127.
 __device__ __forceinline__ signed char quantize_lane(float value, int rule, void* scales, unsigned long long scale_index,
                                                      unsigned int lane)
 {
@@ -228,7 +228,7 @@ template <int GROUPS, bool DRAFT = false> __global__ __launch_bounds__(256) void
         acc = acc + __shfl_xor(acc, 1);
         const float sum = __shfl(acc, 0);
         // sqrtf is correctly rounded (hipcc's default); __fsqrt_rn maps to the native approximation
-        const float mean = DRAFT && p.rule == 3 ? sum * (1.0f / (float)d) : sum / (float)d;
+        const float mean = p.rule == 3 ? sum * (1.0f / (float)d) : sum / (float)d; // the same where d is a power of two
         const float inverse = 1.0f / sqrtf(mean + p.eps);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
@@ -393,7 +393,7 @@ template <int GROUPS, bool DRAFT = false> __global__ __launch_bounds__(256) void
         acc = acc + __shfl_xor(acc, 1);
         const float sum = __shfl(acc, (int)(lane & ~7u));
         // sqrtf is correctly rounded (hipcc's default); __fsqrt_rn maps to the native approximation
-        const float mean = DRAFT && p.rule == 3 ? sum * (1.0f / (float)D) : sum / (float)D;
+        const float mean = sum / (float)D; // D is a power of two: exact, and rule 3's product with 1 / D the same
         const float inverse = 1.0f / sqrtf(mean + p.eps);
         float w[EPL];
         load_run_as_f32<EPL>(weight, part * EPL, 0, w);
@@ -513,7 +513,7 @@ template <int GROUPS, bool DRAFT = false> __global__ __launch_bounds__(256) void
     void* scales = kind == 1u ? p.k_scales : p.v_scales;
     const unsigned long long scale_index = physical * groups_per_row + head * GROUPS + part / LPG;
     const bool writer = live && place.stored && part % LPG == 0u;
-    float factor; // rule 0: the stored scale as f32 (divide by it); rules 1, 2: 1 / scale (multiply by it)
+    float factor; // rule 0: the stored scale as f32 (divide by it); the others: 1 / scale (multiply by it)
     if (p.rule == 0) {
         const float scale = maximum == 0.0f ? 1.0f : __fmul_rn(maximum, 1.0f / 127.0f);
         const unsigned short encoded = f32_to_bf16_bits(scale);
@@ -522,9 +522,9 @@ template <int GROUPS, bool DRAFT = false> __global__ __launch_bounds__(256) void
         }
         factor = bf16_bits_to_f32(encoded);
     } else {
-        const float scale = maximum > 0.0f ? (DRAFT && p.rule == 3 ? __fmul_rn(maximum, 1.0f / 127.0f) : __fdiv_rn(maximum, 127.0f)) : 1.0f;
+        const float scale = maximum > 0.0f ? (p.rule == 3 ? __fmul_rn(maximum, 1.0f / 127.0f) : __fdiv_rn(maximum, 127.0f)) : 1.0f;
         if (writer) {
-            if (p.rule == 1 || (DRAFT && p.rule == 3)) {
+            if (p.rule != 2) {
                 ((unsigned short*)scales)[scale_index] = f32_to_f16_bits(scale);
             } else {
                 ((float*)scales)[scale_index] = scale;
@@ -595,9 +595,9 @@ __global__ __launch_bounds__(256) void q8g64_append_wide(Q8AppendParams p)
         }
         factor = bf16_bits_to_f32(encoded);
     } else {
-        const float scale = maximum > 0.0f ? __fdiv_rn(maximum, 127.0f) : 1.0f;
+        const float scale = maximum > 0.0f ? (p.rule == 3 ? __fmul_rn(maximum, 1.0f / 127.0f) : __fdiv_rn(maximum, 127.0f)) : 1.0f;
         if (writer) {
-            if (p.rule == 1) {
+            if (p.rule != 2) {
                 ((unsigned short*)p.scales)[scale_index] = f32_to_f16_bits(scale);
             } else {
                 ((float*)p.scales)[scale_index] = scale;

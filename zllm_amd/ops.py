@@ -292,10 +292,11 @@ def draft_layout(parents, kv_lens, row_counts=None):
 
 
 def gqa_draft_prologue(q, k, v, q_norm, k_norm, cos, sin, k_plane, k_scales, v_plane, v_scales, tables, kv_lens, num_heads, num_kv_heads, head_dim,
-                       rotary_dim, block_tokens, positions=None, row_counts=None, eps=1e-6, weight_offset=1.0, rule=capi.QUANT_METAL_GQA, split_half=True,
+                       rotary_dim, block_tokens, positions=None, row_counts=None, eps=1e-6, weight_offset=1.0, rule=capi.QUANT_RECIPROCAL_GQA, split_half=True,
                        q_out_dtype=torch.float32, kv_format=capi.KV_Q8G64, ring_capacity=0):
     """gqa_prologue for the drafted nodes of a batch: q [batch * rows, heads * dim]; node i of sequence b rotates at positions[b, i] and its K
-    and V go to cache token kv_lens[b] + i (zllm_attn_gqa_draft_prologue)."""
+    and V go to cache token kv_lens[b] + i (zllm_attn_gqa_draft_prologue).  By default the Q8g64 rows are those that the formula gives as a torch program on
+    the device, bit for bit; `rule` names that of the cache's other rows where a node must have the bits gqa_prologue (METAL_GQA by default) would write."""
     batch = kv_lens.shape[0]
     nodes = q.shape[0]
     rows = nodes // batch
