@@ -172,3 +172,20 @@ def test_definitions_of_the_cases():
     assert dc.verify(tokens, target, torch.tensor([[0.75, 0.9, 0.5, 0.0]]), None, q, [4]) == [([0, 1], [1, 1])]
     sees, depth = dc.ancestors(torch.tensor([[-1, 0, 1, 0, 3]], dtype=torch.int32), [5])
     assert dc.pack(sees).flatten().tolist() == [1, 3, 7, 9, 25] and depth.flatten().tolist() == [0, 1, 2, 1, 2]
+
+
+def test_distributions_whose_rows_overlap_are_refused():
+    """Rows of stride 0 (one distribution expanded over the nodes) or shorter than the vocabulary: the kernel takes 0 for the vocabulary and would read past them."""
+    from zllm_amd import ops
+
+    vocab = 7
+    one = torch.rand(vocab)
+    for t in (one.expand(4, 3, vocab), torch.rand(4, 1, vocab).expand(4, 3, vocab), torch.rand(1, 3, vocab).expand(4, 3, vocab), torch.rand(20).as_strided((4, 3, vocab), (3, 1, 1)),
+              torch.rand(1, 1).expand(4, 3, 1), torch.rand(4, 3, 2 * vocab)[..., ::2]):
+        with pytest.raises(ValueError, match="probs"):
+            ops._prob_rows(t, "target_probs", 12, t.shape[-1], -1)
+    assert ops._prob_rows(torch.rand(4, 3, vocab), "p", 12, vocab, -1) == vocab
+    assert ops._prob_rows(torch.rand(4, 3, 9)[..., :vocab], "p", 12, vocab, -1) == 9
+    assert ops._prob_rows(one.expand(1, 1, vocab), "p", 1, vocab, -1) == vocab
+    assert ops._prob_rows(torch.rand(12, vocab)[::2].view(2, 3, vocab), "p", 6, vocab, -1) == 2 * vocab
+    assert ops._prob_rows(torch.rand(4, 3, 1), "p", 12, 1, -1) == 1

@@ -357,7 +357,7 @@ def gqa_draft_attention(q, *a, **kw):
 
 
 def _prob_rows(t, name, rows, vocab, device):
-    """A tensor of `rows` distributions, [..., vocab] with evenly spaced rows: its elements from row to row."""
+    """A tensor of `rows` distributions, [..., vocab] with evenly spaced rows that do not overlap: its elements from row to row."""
     if t.dtype not in _DTYPE or t.get_device() != device or t.shape[-1] != vocab or t.numel() != rows * vocab or (vocab > 1 and t.stride(-1) != 1):
         raise ValueError(f"{name} must be {rows} rows of {vocab} f32, bf16 or f16 values on the call's device (got {tuple(t.shape)} {t.dtype} {t.device})")
     if t.is_contiguous():
@@ -366,7 +366,10 @@ def _prob_rows(t, name, rows, vocab, device):
     for (_, outer), (count, inner) in zip(spaced, spaced[1:]):
         if outer != inner * count:
             raise ValueError(f"{name}: rows must be evenly spaced")
-    return spaced[-1][1] if spaced else vocab
+    stride = spaced[-1][1] if spaced else vocab
+    if stride < vocab:
+        raise ValueError(f"{name}: rows must not overlap (expanded tensors: call contiguous() first)")
+    return stride
 
 
 def draft_verify(tokens, target_probs, uniforms, parents=None, draft_probs=None, row_counts=None, workspace=None):
