@@ -189,3 +189,52 @@ def test_distributions_whose_rows_overlap_are_refused():
     assert ops._prob_rows(one.expand(1, 1, vocab), "p", 1, vocab, -1) == vocab
     assert ops._prob_rows(torch.rand(12, vocab)[::2].view(2, 3, vocab), "p", 6, vocab, -1) == 2 * vocab
     assert ops._prob_rows(torch.rand(4, 3, 1), "p", 12, 1, -1) == 1
+
+
+def test_planes_of_other_types_or_widths_are_refused():
+    """A cache's planes against the call's formats: what does not fit would be read or written past its end, or as other values."""
+    from zllm_amd import ops
+
+    codes, f16_scales = torch.zeros(32, 256, dtype=torch.int8), torch.zeros(32, 4, dtype=torch.float16)
+    good = dict(k_plane=codes, k_scales=f16_scales, v_plane=codes, v_scales=f16_scales, num_kv_heads=2, head_dim=128, kv_format=capi.KV_Q8G64, scales=torch.float16, device=-1)
+    check = lambda **bad: ops._cache_planes(**{**good, **bad})
+    assert check() == tuple(t.data_ptr() for t in (codes, f16_scales, codes, f16_scales))
+    assert check(k_plane=codes.view(2, 16, 2, 128), k_scales=f16_scales.view(2, 16, 4))[0] == codes.data_ptr()  # any shape of whole rows
+    assert check(k_plane=None)[0] is None  # the C call names null pointers
+    for name, bad in (("k_scales", f16_scales.bfloat16()), ("v_scales", f16_scales.float()), ("k_plane", codes.half()), ("v_plane", codes.float()),
+                      ("k_plane", torch.zeros(32, 250, dtype=torch.int8)), ("v_plane", codes[:16]), ("k_scales", f16_scales[:, :2].contiguous()), ("v_scales", f16_scales[:31]),
+                      ("k_plane", codes[:, ::2]), ("k_plane", codes[:0])):
+        with pytest.raises(ValueError, match=name[2:]):
+            check(**{name: bad})
+    for scales in (torch.bfloat16, torch.float32):
+        with pytest.raises(ValueError, match="scales"):
+            check(scales=scales)
+    with pytest.raises(ValueError, match="plane"):
+        check(head_dim=192)
+    halves = torch.zeros(32, 256, dtype=torch.float16)
+    f16 = dict(k_plane=halves, k_scales=None, v_plane=halves, v_scales=None, kv_format=capi.KV_F16)
+    assert check(**f16) == (halves.data_ptr(), None, halves.data_ptr(), None)
+    for bad in (halves.bfloat16(), codes, halves.float()):
+        with pytest.raises(ValueError, match="plane"):
+            check(**{**f16, "v_plane": bad})
+    assert [ops._RULE_SCALES[rule] for rule in range(4)] == [torch.bfloat16, torch.float16, torch.float32, torch.float16]
+
+
+def test_commit_planes_are_rows():
+    """[layers, rows, columns] is no plane: its first dimension would be taken for tokens."""
+    from zllm_amd import ops
+
+    for plane in (torch.zeros(2, 8, 4), torch.zeros(8), torch.zeros(8, 4)[:, ::2]):
+        with pytest.raises(ValueError, match="plane"):
+            ops._commit_plane(plane, -1)
+    assert ops._commit_plane(torch.zeros(8, 4, dtype=torch.float16), -1) == 8
+
+
+def test_batches_of_no_sequences():
+    from zllm_amd import ops
+
+    none, tables = torch.zeros(0, dtype=torch.int32), torch.zeros(0, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="rows"):
+        ops.gqa_draft_attention(torch.zeros(5, 128), None, None, None, None, tables, none, None, 1, 1, 128, 16, 1.0, 10)
+    with pytest.raises(ValueError, match="rows"):
+        ops.gqa_draft_prologue(torch.zeros(5, 128), None, None, None, None, None, None, None, None, None, None, tables, none, 1, 1, 128, 0, 16)

@@ -266,6 +266,39 @@ def _plane(t, name, device):
     return t.data_ptr()
 
 
+_CODES, _HALVES = (torch.int8, torch.uint8), (torch.float16,)
+_SCALES = {capi.SCALE_BF16: torch.bfloat16, capi.SCALE_F16: torch.float16, capi.SCALE_F32: torch.float32}
+_RULE_SCALES = {capi.QUANT_ROCM_MLA: torch.bfloat16, capi.QUANT_METAL_GQA: torch.float16, capi.QUANT_CUDA_GQA: torch.float32, capi.QUANT_RECIPROCAL_GQA: torch.float16}
+
+
+def _rows_of(plane, name, cols, dtypes, device):
+    """Address and size of a plane of rows of `cols` elements (None: not given, which the C call says)."""
+    if plane is None:
+        return None, 0
+    count = plane.numel()
+    if plane.dtype not in dtypes or count == 0 or count % cols != 0 or plane.get_device() != device or not plane.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of rows of {cols} {dtypes[0]} on the call's device (got {tuple(plane.shape)} {plane.dtype} {plane.device})")
+    return plane.data_ptr(), count
+
+
+def _scales_of(scales, name, codes, dtype, device):
+    if scales is None:
+        return None
+    if (scales.dtype != dtype and dtype is not None) or (codes != 0 and scales.numel() * 64 != codes) or scales.get_device() != device or not scales.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {dtype}, one for every 64 codes of its plane, on the call's device (got {tuple(scales.shape)} {scales.dtype} {scales.device})")
+    return scales.data_ptr()
+
+
+def _cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, scales, device):
+    """Addresses of a cache's planes: rows of num_kv_heads * head_dim int8 codes with a scale of type `scales` (None: any) per 64, or of f16 values."""
+    cols = max(num_kv_heads * head_dim, 1)
+    if kv_format == capi.KV_F16:
+        return _rows_of(k_plane, "k_plane", cols, _HALVES, device)[0], None, _rows_of(v_plane, "v_plane", cols, _HALVES, device)[0], None
+    k, k_codes = _rows_of(k_plane, "k_plane", cols, _CODES, device)
+    v, v_codes = _rows_of(v_plane, "v_plane", cols, _CODES, device)
+    return k, _scales_of(k_scales, "k_scales", k_codes, scales, device), v, _scales_of(v_scales, "v_scales", v_codes, scales, device)
+
+
 def _current(t, name):
     """The current device, which is where the call's tensors have to be."""
     device = torch.cuda.current_device() if t.is_cuda else -1
@@ -299,7 +332,7 @@ def gqa_draft_prologue(q, k, v, q_norm, k_norm, cos, sin, k_plane, k_scales, v_p
     the device, bit for bit; `rule` names that of the cache's other rows where a node must have the bits gqa_prologue (METAL_GQA by default) would write."""
     batch = kv_lens.shape[0]
     nodes = q.shape[0]
-    rows = nodes // batch
+    rows = nodes // max(batch, 1)
     if rows * batch != nodes or tables.dim() != 2 or tables.shape[0] != batch:
         raise ValueError(f"q has {nodes} rows and tables {tuple(tables.shape)}: not the same number a sequence of {batch}")
     device = _current(q, "q")
@@ -309,8 +342,8 @@ def gqa_draft_prologue(q, k, v, q_norm, k_norm, cos, sin, k_plane, k_scales, v_p
         _values(q, "q", nodes * num_heads * head_dim, device), _values(k, "k", nodes * num_kv_heads * head_dim, device, q.dtype),
         _values(v, "v", nodes * num_kv_heads * head_dim, device, q.dtype), _values(q_norm, "q_norm", head_dim, device, torch.float32),
         _values(k_norm, "k_norm", head_dim, device, torch.float32), _values(cos, "cos", angles * (rotary_dim // 2), device, torch.float32),
-        _values(sin, "sin", angles * (rotary_dim // 2), device, torch.float32), q_out.data_ptr(), _plane(k_plane, "k_plane", device), _plane(k_scales, "k_scales", device),
-        _plane(v_plane, "v_plane", device), _plane(v_scales, "v_scales", device), _words(tables, "tables", batch * tables.shape[1], device),
+        _values(sin, "sin", angles * (rotary_dim // 2), device, torch.float32), q_out.data_ptr(),
+        *_cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, _RULE_SCALES.get(rule), device), _words(tables, "tables", batch * tables.shape[1], device),
         _words(kv_lens, "kv_lens", batch, device), _words(positions, "positions", nodes, device), _words(row_counts, "row_counts", batch, device), batch, rows, num_heads,
         num_kv_heads, head_dim, rotary_dim, angles, tables.shape[1], block_tokens, ring_capacity, eps, weight_offset, _DTYPE[q.dtype], _DTYPE[q_out_dtype],
         kv_format, rule, int(split_half))
@@ -325,19 +358,21 @@ def gqa_draft_attention_args(q, k_plane, k_scales, v_plane, v_scales, tables, kv
     times."""
     batch = kv_lens.shape[0]
     nodes = q.shape[0]
-    rows = nodes // batch
+    rows = nodes // max(batch, 1)
     if rows * batch != nodes or tables.dim() != 2 or tables.shape[0] != batch:
         raise ValueError(f"q has {nodes} rows and tables {tuple(tables.shape)}: not the same number a sequence of {batch}")
     device = _current(q, "q")
     if out is None:
         out = q.new_empty((nodes, num_heads * head_dim), dtype=out_dtype)
     args = capi.GqaDraftAttentionArgs(
-        _values(q, "q", nodes * num_heads * head_dim, device), _plane(k_plane, "k_plane", device), _plane(k_scales, "k_scales", device), _plane(v_plane, "v_plane", device),
-        _plane(v_scales, "v_scales", device), _words(tables, "tables", batch * tables.shape[1], device), _words(kv_lens, "kv_lens", batch, device),
+        _values(q, "q", nodes * num_heads * head_dim, device),
+        *_cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, _SCALES.get(scale_dtype), device), _words(tables, "tables", batch * tables.shape[1], device), _words(kv_lens, "kv_lens", batch, device),
         _words(masks, "masks", nodes * ((rows + 63) // 64), device, _LONG), _words(positions, "positions", nodes, device), _words(row_counts, "row_counts", batch, device),
         _values(out, "out", nodes * num_heads * head_dim, device), None, 0, batch, rows, num_heads, num_kv_heads, head_dim, tables.shape[1], max_kv_len, total_kv_tokens,
         block_tokens, ring_capacity, window, score_scale, softcap, kv_format, scale_dtype, _DTYPE[q.dtype], _DTYPE[out.dtype])
     if gate is not None:
+        if gate.dim() != 2:
+            raise ValueError(f"gate must be [{nodes}, 1 or {num_heads * head_dim}] (got {tuple(gate.shape)})")
         args.gate, args.gate_cols, args.gate_dtype = _values(gate, "gate", nodes * gate.shape[1], device), gate.shape[1], _DTYPE[gate.dtype]
     if workspace is None:
         need = capi.load().zllm_attn_gqa_draft_attention_workspace_bytes(C.byref(args))
@@ -402,6 +437,14 @@ def draft_verify(tokens, target_probs, uniforms, parents=None, draft_probs=None,
     return path, accepted, out_tokens
 
 
+def _commit_plane(t, device):
+    """Bytes of a row of a plane [rows, columns]."""
+    _plane(t, "a plane", device)
+    if t.dim() != 2:
+        raise ValueError(f"a plane must be [rows, columns], a row a token (got {tuple(t.shape)})")
+    return t.shape[1] * t.element_size()
+
+
 class CommitPlanes:
     """The planes of a cache (tensors of one row a token) as zllm_attn_commit_rows reads them: made once, used every step."""
 
@@ -410,12 +453,11 @@ class CommitPlanes:
         if not planes:
             raise ValueError("no planes")
         self.device = _current(planes[0], "a plane")
-        for plane in planes:
-            _plane(plane, "a plane", self.device)
+        row_bytes = [_commit_plane(plane, self.device) for plane in planes]
         if len({t.data_ptr() for t in planes}) != len(planes):
             raise ValueError("a plane is given twice: its rows would move twice")
         self.tensors = planes
-        self.array = (capi.KvPlane * len(planes))(*[capi.KvPlane(t.data_ptr(), t.stride(0) * t.element_size()) for t in planes])
+        self.array = (capi.KvPlane * len(planes))(*[capi.KvPlane(t.data_ptr(), size) for t, size in zip(planes, row_bytes)])
 
 
 def commit_planes(planes):
