@@ -238,3 +238,18 @@ def test_batches_of_no_sequences():
         ops.gqa_draft_attention(torch.zeros(5, 128), None, None, None, None, tables, none, None, 1, 1, 128, 16, 1.0, 10)
     with pytest.raises(ValueError, match="rows"):
         ops.gqa_draft_prologue(torch.zeros(5, 128), None, None, None, None, None, None, None, None, None, None, tables, none, 1, 1, 128, 0, 16)
+
+
+def test_calls_larger_than_a_grid_are_refused():
+    """A grid has fewer than 2^32 threads: sizes just above, for each kernel of a call, end as a refusal that names them before anything is launched."""
+    lib = capi.load()
+    refused(lib.zllm_attn_draft_layout(C.byref(fill(capi.DraftLayoutArgs, batch=1 << 24, rows=256)), None), "too many")
+    refused(lib.zllm_attn_draft_layout(C.byref(fill(capi.DraftLayoutArgs, batch=1 << 26, rows=64)), None), "too many")
+    good = dict(rows=256, num_heads=2, num_kv_heads=1, head_dim=192, rotary_dim=0, table_stride=4, block_tokens=16, eps=1e-6)
+    prologue = lambda **more: lib.zllm_attn_gqa_draft_prologue(C.byref(fill(capi.GqaDraftPrologueArgs, **{**good, **more})), None)
+    refused(prologue(batch=1 << 16), "too many")
+    refused(prologue(batch=1 << 16, head_dim=128, k=FAKE + 2), "too many")  # values that are not 16-byte aligned
+    refused(prologue(batch=1 << 19, head_dim=128), "too many")
+    call = lambda **more: lib.zllm_attn_gqa_draft_attention(C.byref(attention_args(workspace_bytes=1 << 40, **more)), None)
+    refused(call(batch=1 << 21, rows=1, num_heads=8, num_kv_heads=8), "too many")
+    refused(call(batch=1 << 18, rows=256, num_heads=1, num_kv_heads=1, head_dim=256, max_kv_len=0, table_stride=16), "too many")  # the merge

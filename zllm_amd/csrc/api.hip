@@ -1564,6 +1564,9 @@ int zllm_attn_draft_layout(const zllm_draft_layout_args* a, zllm_stream_t stream
     if (((uintptr_t)a->masks & 7u) != 0) {
         return fail(-1, "draft layout: masks must be 8-byte aligned");
     }
+    if ((uint64_t)a->batch * ((a->rows + 63u) / 64u * 64u) > 0xffffffffull) {
+        return fail(-1, "draft layout: %u sequences of %u rows are too many for one call", a->batch, a->rows);
+    }
     const zllm::DraftLayoutParams p{a->parents, a->kv_lens, a->row_counts, (unsigned long long*)a->masks, a->positions, a->batch, a->rows};
     return hip_status(zllm::launch_draft_layout(p, (hipStream_t)stream), "draft layout launch");
 }
@@ -1576,7 +1579,6 @@ int zllm_attn_gqa_draft_prologue(const zllm_gqa_draft_prologue_args* a, zllm_str
     }
     if (a->batch == 0 || a->rows == 0 || a->rows > kMaxDraftRows || (uint64_t)a->batch * a->rows > 0x7fffffffull || a->num_heads == 0 ||
         a->num_kv_heads == 0 || (uint64_t)a->num_heads + 2ull * a->num_kv_heads > 0xffffull ||
-        (uint64_t)a->batch * a->rows * (a->num_heads + 2u * a->num_kv_heads) >= (1ull << 29) || // what a grid takes
         a->head_dim == 0 || a->head_dim % ZLLM_GROUP_SIZE != 0 || a->head_dim > 256 || a->block_tokens == 0 || a->table_stride == 0) {
         return fail(-1, "GQA draft prologue: invalid shape batch=%u rows=%u heads=%u/%u head_dim=%u block_tokens=%u table_stride=%u", a->batch, a->rows,
                     a->num_heads, a->num_kv_heads, a->head_dim, a->block_tokens, a->table_stride);
@@ -1605,6 +1607,9 @@ int zllm_attn_gqa_draft_prologue(const zllm_gqa_draft_prologue_args* a, zllm_str
                               a->head_dim, a->rotary_dim, 0, a->block_tokens, a->ring_capacity, a->eps, a->weight_offset,
                               a->src_dtype, a->q_out_dtype, a->rule, a->split_half,
                               {a->kv_lens, a->row_counts, a->positions, a->rows, a->table_stride, a->rope_table_rows, a->kv_format == ZLLM_KV_F16}};
+    if (zllm::gqa_draft_prologue_groups(p) > zllm::kGridGroups) {
+        return fail(-1, "GQA draft prologue: %u sequences of %u rows are too many for one call", a->batch, a->rows);
+    }
     return hip_status(zllm::launch_gqa_draft_prologue(p, (hipStream_t)stream), "GQA draft prologue launch");
 }
 
@@ -1720,7 +1725,9 @@ int zllm_attn_gqa_draft_attention(const zllm_gqa_draft_attention_args* a, zllm_s
         return fail(-1, "GQA draft attention: gate_cols=%u must be 1 or %u, gate_dtype f32 or bf16", a->gate_cols, a->num_heads * a->head_dim);
     }
     const DraftPlan plan = plan_gqa_draft(a);
-    if (plan.items * plan.pair_tiles * a->num_kv_heads > 0x7fffffffull || (uint64_t)a->batch * a->rows * a->num_heads > 0x7fffffffull) {
+    const uint64_t query_heads = (uint64_t)a->batch * a->rows * a->num_heads;
+    if (plan.items * plan.pair_tiles * a->num_kv_heads > zllm::kGridGroups || query_heads > 0x7fffffffull ||
+        zllm::gqa_draft_merge_groups(query_heads, a->head_dim) > zllm::kGridGroups) {
         return fail(-1, "GQA draft attention: %u sequences of %u rows are too many for one call", a->batch, a->rows);
     }
     if (a->workspace_bytes < plan.total) {

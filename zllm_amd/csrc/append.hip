@@ -716,13 +716,24 @@ hipError_t launch_half_append(const HalfAppendParams& p, hipStream_t stream)
     return hipGetLastError();
 }
 
+// vector loads and stores: every tensor and plane 16-byte aligned (rows are multiples of 64 values)
+static bool prologue_is_wide(const GqaPrologueParams& p)
+{
+    const uintptr_t pointers = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q_out | (uintptr_t)p.k_codes | (uintptr_t)p.v_codes |
+                               (uintptr_t)p.q_norm | (uintptr_t)p.k_norm;
+    return (pointers & 15u) == 0 && p.head_dim != 192u;
+}
+
+unsigned long long gqa_draft_prologue_groups(const GqaPrologueParams& p)
+{
+    const unsigned long long units = (unsigned long long)p.rows * (p.num_heads + 2u * p.num_kv_heads);
+    return prologue_is_wide(p) ? (units + 31) / 32 : (units + 3) / 4;
+}
+
 template <bool DRAFT> static hipError_t launch_prologue(const GqaPrologueParams& p, hipStream_t stream)
 {
     const unsigned long long units = (unsigned long long)p.rows * (p.num_heads + 2u * p.num_kv_heads);
-    // vector loads and stores: every tensor and plane 16-byte aligned (rows are multiples of 64 values)
-    const uintptr_t pointers = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q_out | (uintptr_t)p.k_codes | (uintptr_t)p.v_codes |
-                               (uintptr_t)p.q_norm | (uintptr_t)p.k_norm;
-    if ((pointers & 15u) == 0 && p.head_dim != 192u) {
+    if (prologue_is_wide(p)) {
         const dim3 wide_grid((unsigned int)((units + 31) / 32));
         switch (p.head_dim / 64u) {
         case 1: gqa_prologue_wide<1, DRAFT><<<wide_grid, dim3(256), 0, stream>>>(p); break;

@@ -1036,7 +1036,7 @@ template <int D> void launch_draft_merge(const GqaDraftParams& p, hipStream_t st
     constexpr int kSpread = kAlone >= 8 ? 8 : 4;
     constexpr unsigned int kShared = 256 / (D / 4 * kSpread);
     const unsigned long long units = (unsigned long long)p.batch * p.rows * p.num_heads;
-    const unsigned long long groups = (units + kAlone - 1u) / kAlone;
+    const unsigned long long groups = gqa_draft_merge_groups(units, D);
     if (p.max_chunks >= 16u && groups < 256u) {
         gqa_draft_merge<D, kSpread><<<dim3((unsigned int)((units + kShared - 1u) / kShared)), dim3(256), 0, stream>>>(p);
     } else {
@@ -1063,6 +1063,12 @@ unsigned int gqa_draft_wave_columns(unsigned int pairs, unsigned int head_dim, i
 unsigned int gqa_draft_groups_per_cu(unsigned int head_dim, unsigned int wave_columns, int mode)
 {
     return head_dim <= 128u && wave_columns >= 2u && mode != 2 ? (head_dim == 64u ? 3u : 2u) : 1u;
+}
+
+unsigned long long gqa_draft_merge_groups(unsigned long long units, unsigned int head_dim)
+{
+    const unsigned int alone = 256u / (head_dim / 4u);
+    return (units + alone - 1u) / alone;
 }
 
 hipError_t launch_gqa_draft_attention(const GqaDraftParams& p, int kv_format, hipStream_t stream)

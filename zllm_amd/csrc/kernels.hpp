@@ -205,6 +205,9 @@ struct DraftLayoutParams {
     unsigned int batch, rows;
 };
 
+// Workgroups of 256 threads that one dimension of a grid takes: fewer than 2^32 threads
+constexpr unsigned long long kGridGroups = 0xffffffull;
+
 // A cached length that a kernel reads is taken as at most this: lengths, and their sums with nodes and steps, stay 32-bit
 constexpr unsigned int kDraftMaxTokens = 0x7fffff00u;
 
@@ -299,12 +302,14 @@ hipError_t launch_scatter_rows(const ScatterParams& p, hipStream_t stream);
 hipError_t launch_gqa_prologue(const GqaPrologueParams& p, hipStream_t stream);
 // The same over drafted nodes (GqaPrologueParams::draft)
 hipError_t launch_gqa_draft_prologue(const GqaPrologueParams& p, hipStream_t stream);
+unsigned long long gqa_draft_prologue_groups(const GqaPrologueParams& p); // workgroups that it launches
 hipError_t launch_draft_layout(const DraftLayoutParams& p, hipStream_t stream);
 // Waves of a workgroup that hold pairs of their own; the other factor of four is token groups.
 unsigned int gqa_draft_wave_columns(unsigned int pairs, unsigned int head_dim, int mode);
 // Workgroups that a compute unit holds at once
 unsigned int gqa_draft_groups_per_cu(unsigned int head_dim, unsigned int wave_columns, int mode);
 hipError_t launch_gqa_draft_attention(const GqaDraftParams& p, int kv_format, hipStream_t stream);
+unsigned long long gqa_draft_merge_groups(unsigned long long units, unsigned int head_dim); // workgroups of its merge, for (row, head) pairs of the batch
 hipError_t launch_draft_verify(const DraftVerifyParams& p, hipStream_t stream);
 // `unit` bytes (16, 4, 2 or 1) divide every plane's rows and addresses
 hipError_t launch_commit_rows(const CommitParams& p, unsigned int unit, hipStream_t stream);
