@@ -12,7 +12,8 @@
 //   O^T[dim, pair]   += Vcodes^T . P'_g,   P'_g = p * v_scale_g as f16
 // P' stays inside f16's range for any scale a cache can hold: the exponent of the largest V scale met so far is subtracted from the softmax
 // reference, accumulators and sum carry it and it cancels.  What f16 cannot hold below its normal range is 2^-31 of the largest value met: a row
-// whose own tokens' V scales all lie 2^20 and more below those of tokens that it gives no weight keeps fewer bits.
+// whose own tokens' V scales all lie 2^20 and more below those of tokens that it gives no weight keeps fewer bits of its output, never of the sum of its
+// probabilities (kSumLag; the vote for it costs under 1 %).
 // MODE 0, 16-bit queries and bf16 outputs: the V rows of cached tokens are scaled once in LDS, f16(code * scale), and P is one f16.  Both
 // roundings are 2^-11 of a value, a quarter of the output's own 2^-8 together; against f16 outputs (2^-11) they would be 1.6 times as far from 64 bits as an
 // f32 attention rounded once (measured 3.2e-4 and 2.0e-4, 2-norm).  MODE 1, 16-bit queries and other outputs: codes exact, what f16 drops of P' as a
@@ -35,6 +36,9 @@ namespace {
 
 constexpr unsigned int kDraftThreads = 256;
 constexpr float kValueBias = 14.0f; // of p times V scale: f16 ends at 2^16
+// A folded tile's probabilities are summed as f16 holds them, in steps of 2^(lag - 31) where the tile's largest V scale lies 2^lag below the largest met: up to this
+// lag, 2^-30 a token at most.  The sum does not have V's magnitude in it, so tiles further below are summed before they are rounded.
+constexpr int kSumLag = 2;
 // the exponents (biased) that a window of V scales may have: their powers of two, times the bias and a sum, stay inside f32
 constexpr unsigned int kLeastExponent = 32u, kMostExponent = 247u;
 
@@ -641,19 +645,32 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
         float pr[16];
         if constexpr (FOLDED || PLAIN) {
             // p of a folded tile carries 2^(7 + its exponent - the window), so that p . V' carries what acc carries
-            const float shift = FOLDED ? (float)(7 + exponent - window) - reference : kPBias - reference;
+            const int lag = FOLDED ? window - exponent : 0;
+            const bool far = FOLDED && __any(lag > kSumLag);
+            const float shift = FOLDED ? (float)(far ? 7 : 7 - lag) - reference : kPBias - reference;
             Frag ph[2];
-            float sum = 0.0f;
+            float sum = 0.0f, exact = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                pr[i] = __builtin_amdgcn_exp2f(fmaf(s[i], fac, shift));
+            }
+            if (far) {
+                asm volatile(""); // a branch
+                const float down = ldexpf(1.0f, -lag);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    exact += pr[i];
+                    pr[i] *= down;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                pr[i] = __builtin_amdgcn_exp2f(fmaf(s[i], fac, shift));
-                pr[i + 1] = __builtin_amdgcn_exp2f(fmaf(s[i + 1], fac, shift));
                 const unsigned int word = pack_f16_hw(pr[i], pr[i + 1]);
                 ph[i >> 3].u[(i & 7) >> 1] = word;
                 sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, word), f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false); // what is multiplied is what is summed
             }
             between();
-            run_sum = FOLDED ? fmaf(sum, __uint_as_float((unsigned int)(127 + 7 + 127 - exponent) << 23), run_sum) : run_sum + sum;
+            run_sum = FOLDED ? fmaf(far ? exact : sum, __uint_as_float((unsigned int)(127 + 7 + 127 - (far ? window : exponent)) << 23), run_sum) : run_sum + sum;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
 #pragma unroll
