@@ -3,10 +3,12 @@ import pytest
 import torch
 
 from tests import draft_cases as dc
-from tests.test_gpu_draft import SCALE_CODE, dev, ints
+from tests.test_gpu_draft import SCALE_CODE, dev, ints, run_attention
 from zllm_amd import ops
 
 pytestmark = pytest.mark.gpu
+
+FORMS = [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.float32, torch.float32)]
 
 
 @pytest.mark.parametrize("lag", [1, 3, 8, 12, 16, 20, 40, 120])
@@ -33,3 +35,32 @@ def test_tokens_whose_scales_lie_far_below_the_first_ones(lag, scales, heads):
     got = ops.gqa_draft_attention(dev(c["q"]), dev(c["k"]), dev(c["k_scales"]), dev(c["v"]), dev(c["v_scales"]), dev(c["tables"]), ints([n]), dev(c["masks"]), heads, 1, 128,
                                   page, 128**-0.5, 0, scale_dtype=SCALE_CODE[scales], out_dtype=torch.bfloat16).double().cpu()
     assert ((got.view(2, heads, 128) - want.view(2, 1, 128)).abs() <= bound.view(2, 1, 128)).all()
+
+
+@pytest.mark.parametrize("scales,large", [(torch.float16, 60000.0), (torch.bfloat16, 2.0**20), (torch.bfloat16, 2.0**60), (torch.bfloat16, 2.0**127), (torch.float32, 2.0**60),
+                                          (torch.float32, 3.4e38)])
+@pytest.mark.parametrize("q_dtype,out_dtype", FORMS + [(torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("d,rows,kind", [(128, 6, "chain"), (192, 6, "chain"), (64, 40, "tree")])
+def test_finite_scales_of_tokens_that_only_earlier_rows_see(scales, large, q_dtype, out_dtype, d, rows, kind):
+    """The first tokens in reach of a window are seen by node 0 alone; their scales are the largest a cache holds.  The other rows stay within their bound."""
+    c = dc.attention_case(10, [1000], rows, 8, 2, d, kind=kind, window=700, q_dtype=q_dtype, scales=scales)
+    want, about = dc.attention(c, d**-0.5)
+    bound = dc.attention_bound(c, want, about, out_dtype, out_dtype != torch.bfloat16 or q_dtype == torch.float32)
+    others = c["positions"][0] > 1000
+    slot = dc.physical(c["tables"], 0, [1000 + 1 - 700], c["page"])
+    for sign in (1.0, -1.0):
+        other = dict(c, v_scales=c["v_scales"].clone(), k_scales=c["k_scales"].clone())
+        other["v_scales"][slot] = large * sign
+        for k_large in (False, True):
+            if k_large:
+                other["k_scales"][slot] = large
+            got = run_attention(other, d**-0.5, out_dtype).double().cpu()
+            assert ((got - want).abs() <= bound)[others].all()
+        if out_dtype != torch.float16 and large < 2.0**100:  # the row that sees them, as far as its type holds it
+            other["k_scales"] = c["k_scales"]
+            other["v_values"] = c["v_values"].clone()
+            other["v_values"][slot] = other["v"][slot].double() * other["v_scales"][slot].double().repeat_interleave(64, -1)
+            own, own_about = dc.attention(other, d**-0.5)
+            own_bound = dc.attention_bound(c, own, own_about, out_dtype, out_dtype != torch.bfloat16 or q_dtype == torch.float32)
+            got = run_attention(other, d**-0.5, out_dtype).double().cpu()
+            assert ((got - own).abs() <= own_bound).all()

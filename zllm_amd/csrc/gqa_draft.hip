@@ -270,10 +270,13 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
     auto lowest_of = [&](unsigned int position) __attribute__((always_inline)) -> unsigned int {
         return p.window != 0u && position + 1u > p.window ? min(position + 1u - p.window, kv_len) : 0u; // nodes go by their own positions
     };
-    unsigned int lo = 0u, wave_max_lo = 0u;
+    unsigned int seen_by_all = 0u; // every row of the workgroup sees the cached tokens from here on
     if (p.window != 0u) {
-        lo = lowest_of(position_of(mine.query_row));
-        wave_max_lo = wave_max_u(mine.valid ? lo : 0u);
+        for (unsigned int j = lane; j < 32u * CG; j += 64u) {
+            const unsigned int row = (tile * (32u * CG) + j) / p.group;
+            seen_by_all = max(seen_by_all, row < span.count ? lowest_of(position_of(b * p.rows + row)) : 0u);
+        }
+        seen_by_all = wave_max_u(seen_by_all);
     }
 
     // ---- staging ---------------------------------------------------------------------------------------------------
@@ -282,6 +285,15 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
     const unsigned int head_at = kvh * D * (F16 ? 2u : 1u);
     const unsigned int steps = (end - begin + TT * 32u - 1u) / (TT * 32u);
     const unsigned int main_steps = end <= kv_len ? steps : (max(kv_len, begin) - begin) / (TT * 32u); // of cached tokens alone
+    // `lead` of those hold tokens in front of some row's window.  A tile's V scales are taken as a whole where every row sees all of its tokens, so these steps take their
+    // turn among the ones with nodes, behind the other cached tokens: visit v < main_visits is step v + lead.  (A loop of their own before the others spills up to 112
+    // registers.  Five trees of 94 of 64 / 8 heads under a window of 1,024 68.8 -> 70.5 us, 16 of 8 of 32 / 8 24.4 -> 26.1, without a window no change.)
+    const unsigned int lead = seen_by_all > begin ? min(main_steps, (seen_by_all - begin + TT * 32u - 1u) / (TT * 32u)) : 0u;
+    const unsigned int main_visits = main_steps - lead;
+    auto first_token = [&](unsigned int visit) __attribute__((always_inline)) -> unsigned int {
+        const unsigned int step = visit >= main_steps ? visit : (visit >= main_visits ? visit - main_visits : visit + lead);
+        return begin + step * (TT * 32u);
+    };
     // Physical row of a token, in two steps: nothing is formed from a block-table entry before it is needed.  Tokens past the part repeat its last one.
     struct Place {
         unsigned int entry, offset;
@@ -527,7 +539,7 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             }
         }
     };
-    // TAIL: the tile holds drafted nodes or ends with the part; else all of its tokens are cached ones, and only a window's lower edge masks them
+    // TAIL: the tile holds drafted nodes, tokens in front of a window, or ends with the part; else every row sees all of its tokens, those past the part aside
     auto attend = [&](auto tail, unsigned int buf, unsigned int step, unsigned int tt, unsigned int t0, int tile_exponent, f32x16& s, auto between) __attribute__((always_inline)) {
         constexpr bool TAIL = decltype(tail)::value;
         const unsigned int l = TAIL ? fresh_lane() : lane, h = l >> 5;
@@ -595,11 +607,6 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[i] = seen >> (8 * (i >> 2) + (i & 3)) & 1u ? s[i] : kNegInf;
-            }
-        } else if (t0 < wave_max_lo) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = t0 + 8u * (i >> 2) + 4u * h + (i & 3) >= lo ? s[i] : kNegInf;
             }
         }
         float top = s[0];
@@ -746,9 +753,9 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             Place places[4];
 #pragma unroll
             for (unsigned int step = 0; step < 4u; ++step) {
-                places[step] = look_up(begin + step * (TT * 32u) + slot);
+                places[step] = look_up(first_token(step) + slot);
             }
-            ahead = look_up(begin + 4u * (TT * 32u) + slot);
+            ahead = look_up(first_token(4u) + slot);
 #pragma unroll
             for (unsigned int step = 0; step < 4u; ++step) {
                 lds.rows[step][slot] = bytes_of(places[step]);
@@ -767,12 +774,12 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             store_scales(first[1], 1);
         }
         __syncthreads();
-        store_codes(raw, 0, 0, main_steps != 0u);
+        store_codes(raw, 0, 0, main_visits != 0u);
         load_codes(raw, 1);
         __syncthreads();
         auto turn = [&](unsigned int buf, unsigned int step) __attribute__((always_inline)) {
             if (step + 1u < steps) {
-                store_codes(raw, buf ^ 1u, step + 1u, step + 1u < main_steps);
+                store_codes(raw, buf ^ 1u, step + 1u, step + 1u < main_visits);
             }
             load_codes(raw, step + 2u);
             if (step + 2u < steps) {
@@ -780,12 +787,12 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             }
             load_scales(scale_raw, step + 3u);
             lds.rows[step & 3u][slot] = bytes_of(ahead);
-            ahead = look_up(begin + (step + 5u) * (TT * 32u) + slot);
+            ahead = look_up(first_token(step + 5u) + slot);
             __syncthreads();
         };
         auto body = [&](auto parity, unsigned int step) __attribute__((always_inline)) {
             constexpr unsigned int BUF = decltype(parity)::value;
-            const unsigned int t0 = begin + step * (TT * 32u) + tg * (NT * 32u);
+            const unsigned int t0 = begin + (step + lead) * (TT * 32u) + tg * (NT * 32u);
             if (wave_valid && t0 < end) {
                 Frag kf[AHEAD ? kFirstK : 1];
                 int exponents[NT];
@@ -811,19 +818,19 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             turn(BUF, step);
         };
         unsigned int step = 0;
-        for (; step + 1u < main_steps; step += 2u) {
+        for (; step + 1u < main_visits; step += 2u) {
             body(std::integral_constant<unsigned int, 0>{}, step);
             body(std::integral_constant<unsigned int, 1>{}, step + 1u);
         }
-        if (step < main_steps) {
+        if (step < main_visits) {
             body(std::integral_constant<unsigned int, 0>{}, step);
             ++step;
         }
-        // the steps with drafted nodes, a tile at a time through one piece of code
+        // the steps with drafted nodes, and those in front of a window, a tile at a time through one piece of code
         for (; step < steps; ++step) {
 #pragma unroll 1
             for (int j = 0; j < NT; ++j) {
-                const unsigned int t0 = begin + step * (TT * 32u) + (tg * NT + j) * 32u;
+                const unsigned int t0 = first_token(step) + (tg * NT + j) * 32u;
                 if (wave_valid && t0 < end) {
                     f32x16 s;
                     Frag none[AHEAD ? kFirstK : 1];
