@@ -64,3 +64,38 @@ def test_finite_scales_of_tokens_that_only_earlier_rows_see(scales, large, q_dty
             own_bound = dc.attention_bound(c, own, own_about, out_dtype, out_dtype != torch.bfloat16 or q_dtype == torch.float32)
             got = run_attention(other, d**-0.5, out_dtype).double().cpu()
             assert ((got - own).abs() <= own_bound).all()
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", FORMS)
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("rows", [8, 40])
+def test_f16_rows_that_a_node_does_not_see_may_be_anything(q_dtype, out_dtype, d, rows):
+    """Values that are no numbers in the K and V row of one leaf, and of the first token in a window's reach: rows that do not see them keep their bits, and those
+    that do have no number in the dimensions where V has none."""
+    c = dc.attention_case(9, [50], rows, 8, 2, d, fmt="f16", kind="star", q_dtype=q_dtype)
+    want = run_attention(c, d**-0.5, out_dtype).view(rows, 8, d)
+    slot = dc.physical(c["tables"], 0, [50 + 5], c["page"])
+    keep = [i for i in range(rows) if i != 5]
+    dims = [3, d - 1, d + 64]
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        other = dict(c, v=c["v"].clone())
+        other["v"][slot, dims] = bad
+        got = run_attention(other, d**-0.5, out_dtype).view(rows, 8, d)
+        assert torch.equal(got[keep], want[keep])
+        number = torch.isfinite(got[5])
+        assert not number[:4, [3, d - 1]].any() and not number[4:, 64].any()
+        number[:4, [3, d - 1]], number[4:, 64] = True, True
+        assert number.all()
+        other = dict(other, k=c["k"].clone())
+        other["k"][slot] = bad
+        assert torch.equal(run_attention(other, d**-0.5, out_dtype).view(rows, 8, d)[keep], want[keep])
+    c = dc.attention_case(9, [1000, 30], rows, 8, 2, d, fmt="f16", kind="tree", q_dtype=q_dtype, window=700, counts=[rows, rows - 3])
+    want = run_attention(c, d**-0.5, out_dtype).view(2, rows, 8, d)
+    slot = dc.physical(c["tables"], 0, [1000 + 1 - 700], c["page"])
+    keep = (c["positions"][0] > 1000).cuda()
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        other = dict(c, v=c["v"].clone(), k=c["k"].clone())
+        other["v"][slot], other["k"][slot] = bad, bad
+        got = run_attention(other, d**-0.5, out_dtype).view(2, rows, 8, d)
+        assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1], want[1])
+        assert not torch.isfinite(got[0, 0]).any()

@@ -121,6 +121,9 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
     struct Lds {
         Scales scales[F16 ? 1 : 4];
         unsigned long long rows[4][TT * 32];
+        // f16 rows off the main loop: a bit per V value that is no number (a zero stands in its place), and one more than the last step that has any
+        unsigned char odd[2][F16 ? TT : 1][F16 ? 32 : 1][F16 ? D / 8 : 4];
+        unsigned int odd_step[2][F16 ? TT : 1];
         __align__(16) unsigned char k[2][TT][32 * kKRow<D>];
         __align__(16) unsigned char v[2][TT][32 * kRow];
     };
@@ -390,6 +393,7 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             }
         }
     };
+    // fold: a step of the main loop
     auto store_codes = [&](const u32x4 (&raw)[TT][NU], unsigned int buf, unsigned int step, bool fold) __attribute__((always_inline)) {
         unsigned int v_scales[FOLD ? TT : 1][FOLD ? NU : 1]; // all of them before the codes are waited for
         if constexpr (FOLD) {
@@ -419,7 +423,27 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
                 constexpr unsigned int kWide = F16 ? 16u : 32u; // bytes a unit takes in LDS
                 unsigned char* to = is_v ? &lds.v[buf][t][r * kRow + ((c * kWide) ^ (v_block_swap<D>(r) << 6))] : &lds.k[buf][t][r * kKRow<D> + c * kWide];
                 if constexpr (F16) {
-                    *(u32x4*)to = raw[t][j];
+                    u32x4 word = raw[t][j];
+                    if (is_v && !fold) {
+                        unsigned int odd = 0u;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) { // an exponent of ones carries into the sign
+                            odd |= (word[w] & 0x7c007c00u) + 0x04000400u;
+                        }
+                        odd &= 0x80008000u;
+                        if (odd != 0u) {
+                            odd = 0u;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const unsigned int bad = ((word[w] & 0x7c007c00u) + 0x04000400u) >> 15 & 0x00010001u;
+                                word[w] &= ~(bad * 0xffffu);
+                                odd |= ((bad | bad >> 15) & 3u) << (2 * w);
+                            }
+                            lds.odd_step[buf][t] = step + 1u;
+                        }
+                        lds.odd[buf][t][r][c] = (unsigned char)odd;
+                    }
+                    *(u32x4*)to = word;
                 } else {
                     u32x4 half[2];
 #pragma unroll
@@ -539,6 +563,26 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             }
         }
     };
+    // Rows that see a token with V values that are no numbers have none in those dimensions, and zeros in their place keep them from the rows that do not (a weight of
+    // zero does not: zero times infinity).  Looking for them costs the f16 window case (4 x 12 rows, 16 / 8 heads of 256, a few steps a workgroup) 22.7 -> 24.0 us.
+    auto mark_odd = [&](unsigned int buf, unsigned int tt, unsigned int seen) __attribute__((always_inline)) {
+        if constexpr (F16) {
+            const unsigned int h = fresh_lane() >> 5;
+            const unsigned int half = (seen & 0x0f0f0f0fu) << (4u * h), tokens = half | (unsigned int)__shfl_xor((int)half, 32);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                unsigned int hit = 0u; // a bit per dim of the tile
+#pragma unroll 1
+                for (unsigned int token = 0; token < 32u; ++token) {
+                    hit |= (tokens >> token & 1u) != 0u ? *(const unsigned int*)&lds.odd[buf][F16 ? tt : 0u][F16 ? token : 0u][t * 4] : 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    acc[t][i] = hit >> (8u * (i >> 2) + 4u * h + (i & 3)) & 1u ? __builtin_nanf("") : acc[t][i];
+                }
+            }
+        }
+    };
     // TAIL: the tile holds drafted nodes, tokens in front of a window, or ends with the part; else every row sees all of its tokens, those past the part aside
     auto attend = [&](auto tail, unsigned int buf, unsigned int step, unsigned int tt, unsigned int t0, int tile_exponent, f32x16& s, auto between) __attribute__((always_inline)) {
         constexpr bool TAIL = decltype(tail)::value;
@@ -602,6 +646,11 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
                     const int node = first_node + 8 * (i >> 2) + (int)(4u * h) + (i & 3);
                     const bool near = node < 0 || max(at[i], kv_len) + p.window > position;
                     seen &= near ? ~0u : ~(1u << (8 * (i >> 2) + (i & 3)));
+                }
+            }
+            if constexpr (F16) {
+                if (__builtin_amdgcn_readfirstlane(lds.odd_step[buf][tt]) == step + 1u) {
+                    mark_odd(buf, tt, seen);
                 }
             }
 #pragma unroll
@@ -762,6 +811,9 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
             }
         }
         __syncthreads();
+        if (F16 && tid < 2u * TT) {
+            lds.odd_step[tid / TT][F16 ? tid % TT : 0u] = 0u;
+        }
         {
             unsigned int first[2][G];
             load_scales(first[0], 0);
