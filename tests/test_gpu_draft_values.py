@@ -99,3 +99,25 @@ def test_f16_rows_that_a_node_does_not_see_may_be_anything(q_dtype, out_dtype, d
         got = run_attention(other, d**-0.5, out_dtype).view(2, rows, 8, d)
         assert torch.equal(got[0][keep], want[0][keep]) and torch.equal(got[1], want[1])
         assert not torch.isfinite(got[0, 0]).any()
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", FORMS)
+@pytest.mark.parametrize("fmt", ["q8", "f16"])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_scores_that_are_no_numbers(q_dtype, out_dtype, fmt, softcap):
+    """A row that sees a K row that holds no number, or whose query holds none, gives none, with a soft cap too; the other rows keep their bits."""
+    c = dc.attention_case(9, [50], 8, 8, 2, 128, fmt=fmt, kind="star", q_dtype=q_dtype)
+    want = run_attention(c, 128**-0.5, out_dtype, softcap)
+    slot = dc.physical(c["tables"], 0, [50 + 5], c["page"])
+    name = "k_scales" if fmt == "q8" else "k"
+    other = {**c, name: c[name].clone()}
+    other[name][slot] = float("nan")
+    other["q"] = c["q"].clone()
+    other["q"][2] = float("nan")
+    got = run_attention(other, 128**-0.5, out_dtype, softcap)
+    keep = [0, 1, 3, 4, 6, 7]
+    assert torch.equal(got[keep], want[keep])
+    assert torch.isnan(got[[2, 5]]).all()
+    cached = {**c, name: c[name].clone()}
+    cached[name][dc.physical(c["tables"], 0, [7], c["page"])] = float("nan")
+    assert torch.isnan(run_attention(cached, 128**-0.5, out_dtype, softcap)).all()

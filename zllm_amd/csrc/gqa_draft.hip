@@ -608,8 +608,9 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float y = s[i] * mult * inv_cap;
-                s[i] = EXACT ? cap_log2 * soft_tanh(y)
-                             : cap_log2 * fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fminf(y * (2.0f * kLog2e), 126.0f)) + 1.0f), 1.0f);
+                // a score that is no number stays one; past f32's range the power is infinite, its reciprocal zero
+                s[i] = EXACT ? (y == y ? cap_log2 * soft_tanh(y) : y)
+                             : cap_log2 * fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * kLog2e)) + 1.0f), 1.0f);
             }
         }
         unsigned int seen = ~0u; // TAIL: bit 8 (i / 4) + i % 4 for element i
