@@ -121,3 +121,17 @@ def test_scores_that_are_no_numbers(q_dtype, out_dtype, fmt, softcap):
     cached = {**c, name: c[name].clone()}
     cached[name][dc.physical(c["tables"], 0, [7], c["page"])] = float("nan")
     assert torch.isnan(run_attention(cached, 128**-0.5, out_dtype, softcap)).all()
+
+
+@pytest.mark.parametrize("window", [1, 40, 2**31 - 256])
+def test_positions_at_the_end_of_their_range(window):
+    """Nodes at 2^32 - 1 and just before it: a window that does not reach back to the cached tokens holds none of them."""
+    c = dc.attention_case(11, [100, 37], 9, 8, 2, 128, window=window, kind="chain")
+    c["positions"] = c["positions"].long()
+    c["positions"][0] += 2**32 - 1 - 100 - 8
+    c["positions"][1, 4:] = 2**32 - 1
+    scale = 128**-0.5
+    want, about = dc.attention(c, scale)
+    for out_dtype in (torch.bfloat16, torch.float32):
+        got = run_attention(c, scale, out_dtype, positions=dev(c["positions"].to(torch.int32))).double().cpu()
+        assert ((got - want).abs() <= dc.attention_bound(c, want, about, out_dtype, out_dtype != torch.bfloat16)).all()

@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
 
     // cached tokens [lo, kv_len) are visible to the pair's row; nodes by its mask
     auto lowest_of = [&](unsigned int position) __attribute__((always_inline)) -> unsigned int {
-        return p.window != 0u && position + 1u > p.window ? min(position + 1u - p.window, kv_len) : 0u; // nodes go by their own positions
+        return p.window != 0u && position >= p.window ? min(position - p.window + 1u, kv_len) : 0u; // nodes go by their own positions
     };
     unsigned int seen_by_all = 0u; // every row of the workgroup sees the cached tokens from here on
     if (p.window != 0u) {
@@ -645,7 +645,8 @@ __global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void g
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int node = first_node + 8 * (i >> 2) + (int)(4u * h) + (i & 3);
-                    const bool near = node < 0 || max(at[i], kv_len) + p.window > position;
+                    const unsigned int its = max(at[i], kv_len); // positions may be the largest there are: no sums
+                    const bool near = node < 0 || its >= position || position - its < p.window;
                     seen &= near ? ~0u : ~(1u << (8 * (i >> 2) + (i & 3)));
                 }
             }
