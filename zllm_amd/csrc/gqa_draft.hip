@@ -81,14 +81,19 @@ __device__ __forceinline__ float half_wave_max(float v)
     return fmaxf(__uint_as_float(rows.x), __uint_as_float(rows.y));
 }
 
-// How an instantiation runs.  kPerCu: workgroups a CU holds, two where registers and LDS allow (one: 155 -> 215, 124 -> 202, 177 -> 239 us for
+// Workgroups that a compute unit holds at once: what the launch bounds ask for, and what the plan of a call counts with
+constexpr unsigned int groups_per_cu(unsigned int head_dim, unsigned int wave_columns, int mode)
+{
+    return head_dim <= 128u && wave_columns >= 2u && mode != 2 ? (head_dim == 64u ? 3u : 2u) : 1u;
+}
+
+// How an instantiation runs.  groups_per_cu: two where registers and LDS allow (one: 155 -> 215, 124 -> 202, 177 -> 239 us for
 // the calls above), three at D 64 (two: 17 trees of 59, 32 / 8, at 5,584 tokens 177 -> 183; four spill: 191).  kTiles: tiles of 32 tokens a wave
 // takes a step, two with four column waves, which have no token groups (one: 128 -> 143, 178 -> 196; D 192, 15 trees of up to 48 of 24 / 4 heads, 143 ->
 // 158).  kAhead: matrix operands read a phase before they are needed, where registers are left for them (D 192 without: 137 -> 143; D 256, 36
 // trees of 9 of 16 / 2 at 12,621 tokens 247 -> 260; f16 outputs at D 256, 7 trees of 19 at 20,085 tokens, 200 -> 223).
 template <int D, bool F16, int CG, int MODE> struct DraftShape {
     static constexpr int kGroups = 4 / CG; // groups of waves, each with its own tokens
-    static constexpr int kPerCu = D <= 128 && CG >= 2 && MODE != 2 ? (D == 64 ? 3 : 2) : 1;
     static constexpr int kTiles = CG == 4 && MODE != 2 ? 2 : 1;
     static constexpr int kStepTiles = kGroups * kTiles;
     static constexpr int kUnits = D * (F16 ? 2 : 1) / 64; // 16-byte loads a thread, per 32 tokens of K and V
@@ -97,7 +102,7 @@ template <int D, bool F16, int CG, int MODE> struct DraftShape {
 
 // SCALE32: the cache's scales have 32 bits, else 16.
 template <int D, bool F16, int CG, int MODE, bool SCALE32>
-__global__ __launch_bounds__(256, (DraftShape<D, F16, CG, MODE>::kPerCu)) void gqa_draft_partial(GqaDraftParams p)
+__global__ __launch_bounds__(256, (groups_per_cu(D, CG, MODE))) void gqa_draft_partial(GqaDraftParams p)
 {
     using Shape = DraftShape<D, F16, CG, MODE>;
     constexpr int TG = Shape::kGroups, NT = Shape::kTiles, TT = Shape::kStepTiles;
@@ -1140,7 +1145,7 @@ unsigned int gqa_draft_wave_columns(unsigned int pairs, unsigned int head_dim, i
 
 unsigned int gqa_draft_groups_per_cu(unsigned int head_dim, unsigned int wave_columns, int mode)
 {
-    return head_dim <= 128u && wave_columns >= 2u && mode != 2 ? (head_dim == 64u ? 3u : 2u) : 1u;
+    return groups_per_cu(head_dim, wave_columns, mode);
 }
 
 unsigned long long gqa_draft_merge_groups(unsigned long long units, unsigned int head_dim)
