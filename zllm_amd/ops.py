@@ -307,6 +307,16 @@ def _current(t, name):
     return device
 
 
+def _sequences(q, tables):
+    """The device, q's rows, the sequences, rows a sequence and pages a table of a call on q [batch * rows, ...] and tables [batch, pages]."""
+    nodes, shape = q.shape[0], tables.shape
+    batch = shape[0]
+    rows = nodes // max(batch, 1)
+    if rows * batch != nodes or len(shape) != 2:
+        raise ValueError(f"q has {nodes} rows and tables {tuple(shape)}: not the same number of rows a sequence")
+    return _current(q, "q"), nodes, batch, rows, shape[1]
+
+
 def _stream_of(device):
     return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(device)
 
@@ -330,12 +340,7 @@ def gqa_draft_prologue(q, k, v, q_norm, k_norm, cos, sin, k_plane, k_scales, v_p
     """gqa_prologue for the drafted nodes of a batch: q [batch * rows, heads * dim]; node i of sequence b rotates at positions[b, i] and its K
     and V go to cache token kv_lens[b] + i (zllm_attn_gqa_draft_prologue).  By default the Q8g64 rows are those that the formula gives as a torch program on
     the device, bit for bit; `rule` names that of the cache's other rows where a node must have the bits gqa_prologue (METAL_GQA by default) would write."""
-    batch = kv_lens.shape[0]
-    nodes = q.shape[0]
-    rows = nodes // max(batch, 1)
-    if rows * batch != nodes or tables.dim() != 2 or tables.shape[0] != batch:
-        raise ValueError(f"q has {nodes} rows and tables {tuple(tables.shape)}: not the same number a sequence of {batch}")
-    device = _current(q, "q")
+    device, nodes, batch, rows, stride = _sequences(q, tables)
     q_out = q.new_empty((nodes, num_heads * head_dim), dtype=q_out_dtype)
     angles = 0 if cos is None else cos.shape[0]
     args = capi.GqaDraftPrologueArgs(
@@ -343,9 +348,9 @@ def gqa_draft_prologue(q, k, v, q_norm, k_norm, cos, sin, k_plane, k_scales, v_p
         _values(v, "v", nodes * num_kv_heads * head_dim, device, q.dtype), _values(q_norm, "q_norm", head_dim, device, torch.float32),
         _values(k_norm, "k_norm", head_dim, device, torch.float32), _values(cos, "cos", angles * (rotary_dim // 2), device, torch.float32),
         _values(sin, "sin", angles * (rotary_dim // 2), device, torch.float32), q_out.data_ptr(),
-        *_cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, _RULE_SCALES.get(rule), device), _words(tables, "tables", batch * tables.shape[1], device),
+        *_cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, _RULE_SCALES.get(rule), device), _words(tables, "tables", batch * stride, device),
         _words(kv_lens, "kv_lens", batch, device), _words(positions, "positions", nodes, device), _words(row_counts, "row_counts", batch, device), batch, rows, num_heads,
-        num_kv_heads, head_dim, rotary_dim, angles, tables.shape[1], block_tokens, ring_capacity, eps, weight_offset, _DTYPE[q.dtype], _DTYPE[q_out_dtype],
+        num_kv_heads, head_dim, rotary_dim, angles, stride, block_tokens, ring_capacity, eps, weight_offset, _DTYPE[q.dtype], _DTYPE[q_out_dtype],
         kv_format, rule, int(split_half))
     capi.check(capi.load().zllm_attn_gqa_draft_prologue(C.byref(args), _stream_of(device)))
     return q_out
@@ -356,19 +361,14 @@ def gqa_draft_attention_args(q, k_plane, k_scales, v_plane, v_scales, tables, kv
                              scale_dtype=capi.SCALE_F16, out_dtype=torch.float32, out=None, workspace=None, total_kv_tokens=0, gate=None):
     """The argument block of zllm_attn_gqa_draft_attention, the output tensor and the workspace tensor: for callers that launch the same call many
     times."""
-    batch = kv_lens.shape[0]
-    nodes = q.shape[0]
-    rows = nodes // max(batch, 1)
-    if rows * batch != nodes or tables.dim() != 2 or tables.shape[0] != batch:
-        raise ValueError(f"q has {nodes} rows and tables {tuple(tables.shape)}: not the same number a sequence of {batch}")
-    device = _current(q, "q")
+    device, nodes, batch, rows, stride = _sequences(q, tables)
     if out is None:
         out = q.new_empty((nodes, num_heads * head_dim), dtype=out_dtype)
     args = capi.GqaDraftAttentionArgs(
         _values(q, "q", nodes * num_heads * head_dim, device),
-        *_cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, _SCALES.get(scale_dtype), device), _words(tables, "tables", batch * tables.shape[1], device), _words(kv_lens, "kv_lens", batch, device),
+        *_cache_planes(k_plane, k_scales, v_plane, v_scales, num_kv_heads, head_dim, kv_format, _SCALES.get(scale_dtype), device), _words(tables, "tables", batch * stride, device), _words(kv_lens, "kv_lens", batch, device),
         _words(masks, "masks", nodes * ((rows + 63) // 64), device, _LONG), _words(positions, "positions", nodes, device), _words(row_counts, "row_counts", batch, device),
-        _values(out, "out", nodes * num_heads * head_dim, device), None, 0, batch, rows, num_heads, num_kv_heads, head_dim, tables.shape[1], max_kv_len, total_kv_tokens,
+        _values(out, "out", nodes * num_heads * head_dim, device), None, 0, batch, rows, num_heads, num_kv_heads, head_dim, stride, max_kv_len, total_kv_tokens,
         block_tokens, ring_capacity, window, score_scale, softcap, kv_format, scale_dtype, _DTYPE[q.dtype], _DTYPE[out.dtype])
     if gate is not None:
         if gate.dim() != 2:
@@ -378,8 +378,10 @@ def gqa_draft_attention_args(q, k_plane, k_scales, v_plane, v_scales, tables, kv
         need = capi.load().zllm_attn_gqa_draft_attention_workspace_bytes(C.byref(args))
         if need == 0:
             raise capi.ZllmAttnError(-1, capi.last_error())
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    args.workspace, args.workspace_bytes = _plane(workspace, "workspace", device), workspace.numel() * workspace.element_size()
+        workspace = q.new_empty(need, dtype=torch.uint8)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need
+    else:
+        args.workspace, args.workspace_bytes = _plane(workspace, "workspace", device), workspace.numel() * workspace.element_size()
     return args, out, workspace
 
 
