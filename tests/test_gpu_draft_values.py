@@ -135,3 +135,17 @@ def test_positions_at_the_end_of_their_range(window):
     for out_dtype in (torch.bfloat16, torch.float32):
         got = run_attention(c, scale, out_dtype, positions=dev(c["positions"].to(torch.int32))).double().cpu()
         assert ((got - want).abs() <= dc.attention_bound(c, want, about, out_dtype, out_dtype != torch.bfloat16)).all()
+
+
+
+@pytest.mark.parametrize("gate_cols", [1, 8 * 128])
+def test_gates_of_rows_that_give_zeros(gate_cols):
+    """Nodes that are not there, and rows that see nothing, give zeros whatever their gates hold."""
+    c = dc.attention_case(8, [0, 90], 5, 8, 2, 128, counts=[3, 2], empty=[(0, 1)])
+    gate = torch.zeros(10, gate_cols)
+    want = run_attention(c, 128**-0.5, torch.bfloat16, gate=dev(gate))
+    zeros = [1, 3, 4, 7, 8, 9]
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        gate[zeros] = bad
+        got = run_attention(c, 128**-0.5, torch.bfloat16, gate=dev(gate))
+        assert torch.equal(got, want) and (got[zeros] == 0).all()

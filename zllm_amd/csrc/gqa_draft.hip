@@ -1062,7 +1062,7 @@ template <int D, int SPREAD> __global__ __launch_bounds__(256) void gqa_draft_me
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     f32x4 v = sum * inv;
-    if (p.gate != nullptr) {
+    if (p.gate != nullptr && total != 0.0f) { // a row of zeros stays one, whatever its gate holds
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             v[e] = gated(v[e], p.gate, p.gate_cols, p.gate_dtype, query_row, head * D + quad * 4u + e);
