@@ -149,3 +149,25 @@ def test_gates_of_rows_that_give_zeros(gate_cols):
         gate[zeros] = bad
         got = run_attention(c, 128**-0.5, torch.bfloat16, gate=dev(gate))
         assert torch.equal(got, want) and (got[zeros] == 0).all()
+
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [4, 20, 50])
+@pytest.mark.parametrize("power", [40, 70, 110])
+def test_large_scales_behind_scales_of_zero(out_dtype, heads, power):
+    """V rows of zeros (a stored scale of zero), then one row with a scale of 2^power, in one part: the rows of zeros keep their share of the normaliser."""
+    n, page = 320, 16
+    c = dc.attention_case(3, [n], 2, heads, 1, 128, scales=torch.bfloat16)
+    last = dc.physical(c["tables"], 0, [n - 1], page)
+    c["k_scales"].fill_(2.0**-20)
+    c["v_scales"].fill_(0.0)
+    c["v_scales"][last] = 2.0**power
+    c["v"][last] = 100
+    for name in ("k", "v"):
+        c[name][c[name] == -128] = 0
+        c[name + "_values"] = (c[name].view(-1, 2, 64).double() * c[name + "_scales"].double()[..., None]).view(c[name].shape)
+    want, about = dc.attention(c, 128**-0.5)
+    got = ops.gqa_draft_attention(dev(c["q"]), dev(c["k"]), dev(c["k_scales"]), dev(c["v"]), dev(c["v_scales"]), dev(c["tables"]), ints([n]), dev(c["masks"]), heads, 1, 128,
+                                  page, 128**-0.5, 0, scale_dtype=SCALE_CODE[torch.bfloat16], out_dtype=out_dtype).double().cpu()
+    assert ((got - want).abs() <= dc.attention_bound(c, want, about, out_dtype, out_dtype != torch.bfloat16)).all()

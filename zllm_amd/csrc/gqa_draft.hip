@@ -695,10 +695,11 @@ __global__ __launch_bounds__(256, (groups_per_cu(D, CG, MODE))) void gqa_draft_p
         // scales follow in the product.
         if (__any((FOLDED || PLAIN ? top - run_max > kSlack : top > run_max) || now != window)) {
             const float new_max = fmaxf(run_max, halves_max(top));
-            const float alpha = ldexpf(__builtin_amdgcn_exp2f(run_max - (new_max == kNegInf ? 0.0f : new_max)), window - now);
+            const float keep = __builtin_amdgcn_exp2f(run_max - (new_max == kNegInf ? 0.0f : new_max));
+            const float alpha = ldexpf(keep, window - now);
+            run_sum = ldexpf(run_sum * keep, window - now); // 2^(window - now) alone may lie below f32's range
             run_max = new_max;
             window = now;
-            run_sum *= alpha;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 acc[t] *= alpha;
