@@ -171,3 +171,20 @@ def test_large_scales_behind_scales_of_zero(out_dtype, heads, power):
     got = ops.gqa_draft_attention(dev(c["q"]), dev(c["k"]), dev(c["k_scales"]), dev(c["v"]), dev(c["v_scales"]), dev(c["tables"]), ints([n]), dev(c["masks"]), heads, 1, 128,
                                   page, 128**-0.5, 0, scale_dtype=SCALE_CODE[torch.bfloat16], out_dtype=out_dtype).double().cpu()
     assert ((got - want).abs() <= dc.attention_bound(c, want, about, out_dtype, out_dtype != torch.bfloat16)).all()
+
+
+
+@pytest.mark.parametrize("q_dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("heads", [4, 20, 50])
+@pytest.mark.parametrize("power", [24, 30, 60, 100])
+def test_scores_far_from_zero(q_dtype, out_dtype, heads, power):
+    """Queries up to the end of their range: scores are numbers, and so are the outputs, those of the largest score alone."""
+    c = dc.attention_case(11, [200], 6, heads, 1, 128, q_dtype=q_dtype)
+    about = dc.attention(c, 128**-0.5)[1]
+    c["q"][2] *= 2.0**power
+    got = run_attention(c, 128**-0.5, out_dtype).double().cpu()
+    right, _ = dc.attention(c, 128**-0.5)
+    keep = [0, 1, 3, 4, 5]
+    assert ((got - right).abs() <= dc.attention_bound(c, right, about, out_dtype, out_dtype != torch.bfloat16 or q_dtype == torch.float32))[keep].all()
+    half = dc.EPS[out_dtype] + 2.0**-9  # the output's rounding; probabilities and V rows as f16
+    assert ((got[2] - right[2]).abs() <= half * right[2].abs() + 2.0**-20).all()

@@ -39,6 +39,7 @@ constexpr float kValueBias = 14.0f; // of p times V scale: f16 ends at 2^16
 // A folded tile's probabilities are summed as f16 holds them, in steps of 2^(lag - 31) where the tile's largest V scale lies 2^lag below the largest met: up to this
 // lag, 2^-30 a token at most.  The sum does not have V's magnitude in it, so tiles further below are summed before they are rounded.
 constexpr int kSumLag = 2;
+constexpr float kFarScore = 16777216.0f; // f32 rounds what is larger by more than a half
 // the exponents (biased) that a window of V scales may have: their powers of two, times the bias and a sum, stay inside f32
 constexpr unsigned int kLeastExponent = 32u, kMostExponent = 247u;
 
@@ -483,6 +484,7 @@ __global__ __launch_bounds__(256, (groups_per_cu(D, CG, MODE))) void gqa_draft_p
     // acc and run_sum carry 2^(kValueBias - exponent of the largest V scale that the pair has met) (f16 rows: 2^kPBias)
     float run_max = kNegInf, run_sum = 0.0f;
     int window = (int)kLeastExponent; // that exponent, biased as f32's
+    bool far_scores = false; // of the wave: a pair's run_max lies past kFarScore
 
     // Operand t, kk of a V tile: dims 32 t + lane % 32, tokens 16 kk + 4 h + {0 .. 3, 8 .. 11}, which are the tokens of elements 8 kk .. of the scores
     auto v_operand = [&](const unsigned char* vt, unsigned int l, int t, int kk) __attribute__((always_inline)) -> f16x8 {
@@ -704,8 +706,22 @@ __global__ __launch_bounds__(256, (groups_per_cu(D, CG, MODE))) void gqa_draft_p
             for (int t = 0; t < DT; ++t) {
                 acc[t] *= alpha;
             }
+            far_scores = __any(fabsf(run_max) > kFarScore && run_max != kNegInf);
         }
-        const float reference = run_max == kNegInf ? 0.0f : run_max;
+        float reference = run_max == kNegInf ? 0.0f : run_max;
+        // The reference is a rounded product, and what it is subtracted from in a multiply-add is not: far from zero what its rounding left is more than a power of two, and p
+        // would leave f16.  Such pairs' scores are rounded first.
+        if (far_scores) {
+            const bool far = fabsf(reference) > kFarScore;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float rounded = s[i] * fac;
+                asm volatile("" : "+v"(rounded)); // no multiply-add
+                s[i] = far ? rounded - reference : s[i];
+            }
+            fac = far ? 1.0f : fac;
+            reference = far ? 0.0f : reference;
+        }
         float pr[16];
         if constexpr (FOLDED || PLAIN) {
             // p of a folded tile carries 2^(7 + its exponent - the window), so that p . V' carries what acc carries
