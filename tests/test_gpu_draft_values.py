@@ -176,7 +176,7 @@ def test_large_scales_behind_scales_of_zero(out_dtype, heads, power):
 
 @pytest.mark.parametrize("q_dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
 @pytest.mark.parametrize("heads", [4, 20, 50])
-@pytest.mark.parametrize("power", [24, 30, 60, 100])
+@pytest.mark.parametrize("power", [24, 30, 60, 100, 122])
 def test_scores_far_from_zero(q_dtype, out_dtype, heads, power):
     """Queries up to the end of their range: scores are numbers, and so are the outputs, those of the largest score alone."""
     c = dc.attention_case(11, [200], 6, heads, 1, 128, q_dtype=q_dtype)

@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256, (groups_per_cu(D, CG, MODE))) void gqa_draft_p
             }
         }
         amax = halves_max(amax);
-        const unsigned int q_exp = min(max((__float_as_uint(amax) >> 23) & 0xffu, 16u), 240u);
+        const unsigned int q_exp = min(max((__float_as_uint(amax) >> 23) & 0xffu, 16u), 254u);
         const float q_mul = __uint_as_float((262u - q_exp) << 23); // 2^(127 + 8 - q_exp)
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
