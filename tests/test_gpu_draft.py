@@ -755,3 +755,18 @@ def test_prologue_default_rows_are_those_of_a_tensor_program():
             assert torch.equal(one, other)
         if src == torch.bfloat16:  # the two rules do differ here
             assert not torch.equal(results[capi.QUANT_METAL_GQA][1][2], v_codes)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_prologue_lengths_at_the_end_of_their_range(shift):
+    """Nodes of a sequence whose length is no length (-1): none of them has a place in the sequence's pages, the first pages among them."""
+    gen = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(8, 64, generator=gen).cuda() for _ in range(3))
+    codes = [torch.zeros(24 * 64 + 16, dtype=torch.int8, device="cuda")[shift : 24 * 64 + shift].view(24, 64) for _ in range(2)]
+    steps = [torch.zeros(24, 1, dtype=torch.float16, device="cuda") for _ in range(2)]
+    tables = torch.tensor([[0, 1, 2], [5, 4, 3]], dtype=torch.int32)
+    ops.gqa_draft_prologue(q, k, v, None, None, None, None, codes[0], steps[0], codes[1], steps[1], dev(tables), ints([-1, 2]), 1, 1, 64, 0, 4)
+    written = torch.zeros(24, dtype=torch.bool)
+    written[dc.physical(tables, 1, range(2, 6), 4)] = True
+    for plane in codes + steps:
+        assert torch.equal((plane != 0).any(-1).cpu(), written)

@@ -160,11 +160,12 @@ template <bool DRAFT> __device__ __forceinline__ PrologueRow prologue_row(const 
         const unsigned int wanted = p.draft.positions != nullptr ? p.draft.positions[row] : kv_len + i;
         at.rope_row = min(wanted, max(p.draft.rope_table_rows, 1u) - 1u);
         unsigned int token = kv_len + i;
+        const bool counts = token >= kv_len; // a sum that wrapped is no place
         if (p.ring_capacity != 0u) {
             token %= p.ring_capacity;
         }
         const unsigned int page = token / p.block_tokens;
-        at.stored = at.there && page < p.draft.table_stride;
+        at.stored = at.there && counts && page < p.draft.table_stride;
         at.physical = at.stored ? (unsigned long long)p.table[(size_t)b * p.draft.table_stride + page] * p.block_tokens + token % p.block_tokens : 0ull;
     } else {
         const unsigned int position = p.positions != nullptr ? p.positions[0] : p.position;
