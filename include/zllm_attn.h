@@ -607,7 +607,7 @@ ZLLM_API int zllm_attn_gqa_draft_prologue(const zllm_gqa_draft_prologue_args* ar
  * and nodes whose position plus the window exceeds its own (positions are then needed; one below kv_lens[b] counts as
  * kv_lens[b]).  A node that sees nothing, and one that is not there, gives zeros, never NaN.  What a node does not see may hold
  * any values and scales.  Of what it sees, a scale or a K row that is no number leaves it without numbers, an f16 V row with
- * values that are none without those dimensions.  16-bit queries
+ * values that are none without those dimensions.  Products with V are kept to 2^-31 of the largest V value that the node sees.  16-bit queries
  * with bf16 outputs round probabilities and scaled V rows to f16, 2^-11 of a value each; with f16 and f32 outputs the
  * probabilities are carried in two terms, with f32 queries those too. */
 typedef struct zllm_gqa_draft_attention_args {

@@ -20,10 +20,12 @@
 // second term.  MODE 2, f32 queries: what f16 drops of Q' too.
 // Splits leave (partial, maximum, sum) records for gqa_draft_merge.
 //
-// What bounds it.  64 rows of 64 / 8 heads of 128 on 50,000 tokens, 172-180 us: of a SIMD's ~ 360 K cycles vector instructions take 168 K and matrix
-// instructions 100 K, of the CU's LDS its reads and writes 232 K; the two waves a SIMD that the registers allow overlap these in part.  Eight sequences
-// of 5 rows (64 / 8) at 32,768 tokens, 152-166 us: 3.5 TB/s, vector instructions 45 %.  Eight ragged trees of up to 24 rows (32 / 8), 124 us.
-// What carried it, in order (us of the three): V scales folded and requests two steps ahead 430 / 531 / 524 -> 236 / 176 / 227; loads without
+// What bounds it (times of calls in a row, with the merge).  64 rows of 64 / 8 heads of 128 on 50,000 tokens, 163-169 us: of a SIMD's ~ 360 K cycles
+// vector instructions take 168 K and matrix instructions 100 K, of the CU's LDS its reads and writes 232 K; the two waves a SIMD that the registers
+// allow overlap these in part.  Eight sequences of 5 rows (64 / 8) at 32,768 tokens, 160-164 us: 3.4 TB/s, vector instructions 45 %.  Eight ragged
+// trees of up to 24 rows (32 / 8), 122-124 us.
+// What carried it, in order (us of this kernel alone, chains / ragged trees / the wide tree, each in the build it was measured in): V scales folded and
+// requests two steps ahead 430 / 531 / 524 -> 236 / 176 / 227; loads without
 // conditions, which the compiler counts exactly, and nothing waiting for scales or table entries -> 210 / 149 / 194; operands read from LDS a phase
 // ahead -> 187 / 134 / 185; queries formed under the first loads, groups of waves meeting in LDS, requests at a step's end -> 155 / 124 / 177.
 #include <type_traits>
