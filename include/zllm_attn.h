@@ -608,7 +608,7 @@ ZLLM_API int zllm_attn_gqa_draft_prologue(const zllm_gqa_draft_prologue_args* ar
  * kv_lens[b]).  A node that sees nothing, and one that is not there, gives zeros, never NaN.  What a node does not see may hold
  * any values and scales.  Of what it sees, a scale or a K row that is no number leaves it without numbers, an f16 V row with
  * values that are none without those dimensions.  Products with V are kept to 2^-31 of the largest V value that the node sees.  16-bit queries
- * with bf16 outputs round probabilities and scaled V rows to f16, 2^-11 of a value each; with f16 and f32 outputs the
+ * with bf16 outputs round probabilities, scaled V rows and f32 scales to f16, 2^-11 of a value each; with f16 and f32 outputs the
  * probabilities are carried in two terms, with f32 queries those too. */
 typedef struct zllm_gqa_draft_attention_args {
     const void* q;              /* [dev] [batch * rows, num_heads * head_dim], q_dtype */

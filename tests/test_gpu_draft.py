@@ -726,7 +726,7 @@ def test_prologue_default_rows_are_those_of_a_tensor_program():
     norm = (torch.randn(d, generator=gen) * 0.1).cuda()
     for src in (torch.bfloat16, torch.float16, torch.float32):
         q, k, v = torch.randn(3, nodes, cols, generator=gen).to(src).cuda()
-        empty = lambda: [torch.zeros(nodes, cols, dtype=torch.int8, device="cuda"), torch.zeros(nodes, cols // 64, dtype=torch.float16, device="cuda")] * 1
+        empty = lambda: [torch.zeros(nodes, cols, dtype=torch.int8, device="cuda"), torch.zeros(nodes, cols // 64, dtype=torch.float16, device="cuda")]
 
         def drafted(**rule):
             planes = empty() + empty()
